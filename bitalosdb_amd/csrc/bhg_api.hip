@@ -143,7 +143,10 @@ void set_err(bhg_ctx *c, const char *fmt, ...) {
     va_end(ap);
 }
 
+// A failed call is reported here, once: its error is taken out of the runtime's per-thread
+// "last error", which the launches read (hipGetLastError) and would else report as their own.
 int hip_fail(bhg_ctx *c, hipError_t e, const char *what) {
+    (void)hipGetLastError();
     set_err(c, "%s: %s", what, hipGetErrorString(e));
     return e == hipErrorOutOfMemory ? BHG_ENOMEM : BHG_EHIP;
 }
