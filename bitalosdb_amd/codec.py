@@ -95,6 +95,7 @@ class BithashCodec:
         if not torch.cuda.is_available():
             raise B.BhgError("no GPU visible: the bithash codec has no CPU path")
         self.device = torch.device("cuda", device)
+        self._unpinned = set()               # addresses whose host_register the runtime refused
         self.L = B.lib()
         self.ctx = self.L.bhg_create(device, 0)
         if not self.ctx:
@@ -327,10 +328,23 @@ class BithashCodec:
         return st, desc, None, None
 
     def host_register(self, arr):
-        """Pin a host numpy buffer (bhg_host_register) for DMA-rate *_host copies."""
-        B.check(self.ctx, self.L.bhg_host_register(self.ctx, _ptr(arr), arr.nbytes), "bhg_host_register")
+        """Pin a host numpy buffer (bhg_host_register) for DMA-rate *_host copies.  True when it
+        is pinned; False where the runtime refuses to page-lock memory that already exists: the
+        buffer stays pageable and the *_host calls take it all the same, at the pageable rate
+        (memory allocated as pinned, bhg_malloc_host or torch's pin_memory, needs no registration).
+        Pair it with host_unregister either way."""
+        rc = self.L.bhg_host_register(self.ctx, _ptr(arr), arr.nbytes)
+        if rc == B.BHG_EHIP:
+            self._unpinned.add(_ptr(arr))
+            return False
+        B.check(self.ctx, rc, "bhg_host_register")
+        self._unpinned.discard(_ptr(arr))
+        return True
 
     def host_unregister(self, arr):
+        if _ptr(arr) in self._unpinned:      # host_register was refused: nothing to undo
+            self._unpinned.discard(_ptr(arr))
+            return
         B.check(self.ctx, self.L.bhg_host_unregister(self.ctx, _ptr(arr)), "bhg_host_unregister")
 
     # ---- primitives ----

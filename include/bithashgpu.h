@@ -183,7 +183,12 @@ int bhg_decode_batch_host(bhg_ctx *ctx, const uint8_t *src, uint64_t src_len, co
 /* Page-lock (pin) a caller host range, e.g. an mmap'd .bht file, and map it
  * into the device address space (hipHostRegister, mapped + portable): the
  * *_host paths then read it in place (NoCompressor) or copy it by DMA at the
- * link rate instead of through pageable staging.  Unregister before unmapping. */
+ * link rate instead of through pageable staging.  Unregister before unmapping.
+ * BHG_EHIP: the runtime refused to page-lock this memory (some hosts do not
+ * allow it for memory that already exists).  The range is then as it was, not
+ * to be unregistered; the *_host paths take it as pageable memory, with the
+ * same results.  Memory from bhg_malloc_host is page-locked and mapped without
+ * being registered. */
 int bhg_host_register(bhg_ctx *ctx, void *p, uint64_t bytes);
 int bhg_host_unregister(bhg_ctx *ctx, void *p);
 
