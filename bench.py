@@ -405,6 +405,51 @@ def run(a, world, rank, local, dev, codec):
         print(json.dumps(out), flush=True)
 
 
+def pinned_copy(x):
+    """A copy of a numpy array in memory that is allocated page-locked (and mapped into the device)."""
+    t = torch.empty(x.nbytes, dtype=torch.uint8, pin_memory=True)
+    t.numpy()[:] = x.view(np.uint8).reshape(-1)
+    return t.numpy().view(x.dtype)
+
+
+def host_leg(out, leg):
+    """The end-to-end leg is optional: its record goes to out["e2e_host"], and if the host refuses
+    what it needs (page-locked memory, say) the reason stands there and the line is printed all the same."""
+    try:
+        out["e2e_host"] = leg()
+    except (RuntimeError, MemoryError) as e:
+        out["e2e_host"] = {"value": None, "error": "%s: %s" % (type(e).__name__, e)}
+
+
+def time_host(run, warm=2, reps=5):
+    for _ in range(warm):       # warm the ring buffers (the second call still ran ~15 % slow on the box)
+        run()
+    t = time.perf_counter()
+    for _ in range(reps):
+        got = run()
+    return (time.perf_counter() - t) / reps, got
+
+
+def c2_host_leg(codec, host_src, h, d):
+    """End-to-end: host src -> H2D -> kernel -> D2H descriptors (bhg_decode_batch_host; handles are
+    sorted, so the 64 MiB-chunk 3-stream pipeline runs).  Pageable buffers first, then copies of the
+    table bytes and the handle list, and a descriptor buffer, in memory allocated page-locked.
+    d: the device path's descriptors of the same batch."""
+    bufs = (host_src, np.ascontiguousarray(h), np.empty(len(h), dtype=DESC_DT))
+    e2e, ok = {}, True
+    for mode in ("pageable", "pinned"):
+        src, hs, desc = bufs if mode == "pageable" else [pinned_copy(b) for b in bufs]
+        desc.view(np.uint8)[:] = 0xEE
+        s, (got, _, _) = time_host(lambda: codec.decode_host(src, hs, out_desc=desc))
+        e2e[mode] = round(float(h["length"].astype(np.float64).sum()) / s / 2 ** 30, 3)
+        ok = ok and bool(np.array_equal(got["crc"], d["crc"]) and np.array_equal(got["status"], d["status"]))
+    return {"value": e2e["pinned"], "unit": "GiB/s", "pageable": e2e["pageable"], "matches_device_path": ok,
+            "note": "host src (%.2f GB) + handles -> descriptors in host memory, 64 MiB chunks "
+                    "over 3 streams (H2D, decode, D2H overlapped), descriptor buffer reused.  value: "
+                    "src, handles and descriptors in memory allocated page-locked; pageable also "
+                    "given" % (host_src.size / 1e9)}
+
+
 def c2_measure(a, world, rank, local, dev, codec, with_extras):
     """BASELINE configs[1] on this rank's GPU: 1M blocks of its own tables,
     CRC-verify + record decode, K timed steps.  Returns the bench line (dict)."""
@@ -509,36 +554,8 @@ def c2_measure(a, world, rank, local, dev, codec, with_extras):
     }
 
     if rank == 0 and world == 1 and with_extras and not a.no_e2e:
-        # end-to-end: host src -> H2D -> kernel -> D2H descriptors (bhg_decode_batch_host; handles are
-        # sorted, so the 64 MiB-chunk 3-stream pipeline runs).  Pageable first, then the same buffer
-        # page-locked with bhg_host_register (an mmap'd table file pinned once per mapping).
         host_src = src_t.cpu().numpy()
-        from bitalosdb_amd.codec import DESC_DT
-        host_desc = np.empty(n, dtype=DESC_DT)
-        e2e = {}
-        for mode in ("pageable", "pinned"):
-            if mode == "pinned":   # an mmap'd table file, its handle list and a reused descriptor buffer, pinned once
-                codec.host_register(host_src)
-                codec.host_register(host_desc)
-                codec.host_register(h)
-            for _ in range(2):      # warm the ring buffers (the second call still ran ~15 % slow on the box)
-                codec.decode_host(host_src, h, out_desc=host_desc)
-            reps, t = 5, time.perf_counter()
-            for _ in range(reps):
-                got_host, _, _ = codec.decode_host(host_src, h, out_desc=host_desc)
-            e2e_s = (time.perf_counter() - t) / reps
-            e2e[mode] = round(n * L / e2e_s / 2 ** 30, 3)
-            if mode == "pinned":
-                codec.host_unregister(h)
-                codec.host_unregister(host_desc)
-                codec.host_unregister(host_src)
-        host_ok = bool(np.array_equal(got_host["crc"], d["crc"]) and np.array_equal(got_host["status"], d["status"]))
-        out["e2e_host"] = {"value": e2e["pinned"], "unit": "GiB/s", "pageable": e2e["pageable"],
-                           "matches_device_path": host_ok,
-                           "note": "host src (%.2f GB) + handles -> descriptors in host memory, 64 MiB chunks "
-                                   "over 3 streams (H2D, decode, D2H overlapped), descriptor buffer reused.  value: "
-                                   "src, handles and descriptors page-locked (bhg_host_register); pageable also "
-                                   "given" % (host_src.size / 1e9)}
+        host_leg(out, lambda: c2_host_leg(codec, host_src, h, d))
     else:
         host_src = None
 
@@ -816,47 +833,41 @@ def c3_measure(a, world, rank, local, dev, codec, gen, extras):
         out["parity_vs_restatement"] = "bit-exact" if par else "MISMATCH"
         out["valid"] = bool(out["valid"] and par)
     if extras and rank == 0 and world == 1 and not a.no_e2e:
-        # end-to-end: host table bytes -> H2D -> header/CRC pass + scan + snappy -> D2H descriptors, value
-        # offsets and the decoded values (bhg_decode_batch_host; snappy stages the whole src in HBM).
-        # Caller-owned output buffers are reused; pageable first, then page-locked (bhg_host_register).
-        host_src = src.cpu().numpy()
-        ecrc_h = exp_crc.cpu().numpy().view(np.uint32).copy()
-        host_desc = np.empty(n, dtype=DESC_DT)
-        host_vals = np.empty(n * 1024 + 64, dtype=np.uint8)
-        e2e = {}
-        for mode in ("pageable", "pinned"):
-            bufs = (host_src, host_desc, host_vals, h, ecrc_h)
-            if mode == "pinned":
-                for b in bufs:
-                    codec.host_register(b)
-            run = lambda: codec.decode_host(host_src, h, compressor=1, expected_crc=ecrc_h,
-                                            out_desc=host_desc, out_vals=host_vals)
-            run()
-            run()
-            reps, t = 5, time.perf_counter()
-            for _ in range(reps):
-                got_d, got_v, _ = run()
-            e2e_s = (time.perf_counter() - t) / reps
-            e2e[mode] = round(disk / e2e_s / 2 ** 30, 3)
-            if mode == "pinned":
-                for b in bufs[::-1]:
-                    codec.host_unregister(b)
         d_vals = vals.cpu().numpy()
-        nv = got_v.size
-        host_ok = bool(all(np.array_equal(got_d[f], d[f]) for f in d.dtype.names)
-                       and np.array_equal(got_v, d_vals[:nv]))
-        out["e2e_host"] = {"value": e2e["pinned"], "unit": "GiB/s on disk", "pageable": e2e["pageable"],
-                           "decoded_GiBps_pinned": round(e2e["pinned"] * n * 1024 / disk, 3),
-                           "matches_device_path": host_ok,
-                           "note": "host src (%.2f GB) + handles + expected CRCs -> descriptors, value offsets and "
-                                   "%.2f GB of decoded values in host memory: 64 MiB src chunks, chunk k + 1's H2D "
-                                   "under chunk k's values going back (a copy kernel into the mapped out_vals when "
-                                   "it is page-locked, else into page-locked staging that host threads copy on), "
-                                   "caller-owned output buffers reused.  value: "
-                                   "all host buffers page-locked (bhg_host_register); pageable also given"
-                                   % (host_src.size / 1e9, n * 1024 / 1e9)}
-        out["valid"] = bool(out["valid"] and host_ok)
+        host_leg(out, lambda: c3_host_leg(codec, src.cpu().numpy(), h, exp_crc.cpu().numpy().view(np.uint32), d, d_vals))
+        out["valid"] = bool(out["valid"] and out["e2e_host"].get("matches_device_path", True))
     return out
+
+
+def c3_host_leg(codec, host_src, h, exp_crc, d, d_vals):
+    """End-to-end: host table bytes -> H2D -> header/CRC pass + scan + snappy -> D2H descriptors, value
+    offsets and the decoded values (bhg_decode_batch_host).  Caller-owned output buffers are reused;
+    pageable first, then every buffer in memory allocated page-locked.  d, d_vals: the device path's
+    descriptors and values of the same batch."""
+    n = len(h)
+    disk = float(h["length"].astype(np.float64).sum())
+    bufs = (host_src, np.ascontiguousarray(h), exp_crc, np.empty(n, dtype=DESC_DT),
+            np.empty(n * 1024 + 64, dtype=np.uint8))
+    e2e, ok = {}, True
+    for mode in ("pageable", "pinned"):
+        src, hs, ecrc, desc, vals = bufs if mode == "pageable" else [pinned_copy(b) for b in bufs]
+        desc.view(np.uint8)[:] = 0xEE
+        vals[:] = 0xEE
+        s, (got_d, got_v, _) = time_host(lambda: codec.decode_host(src, hs, compressor=1, expected_crc=ecrc,
+                                                                   out_desc=desc, out_vals=vals))
+        e2e[mode] = round(disk / s / 2 ** 30, 3)
+        ok = ok and bool(all(np.array_equal(got_d[f], d[f]) for f in d.dtype.names)
+                         and np.array_equal(got_v, d_vals[:got_v.size]))
+    return {"value": e2e["pinned"], "unit": "GiB/s on disk", "pageable": e2e["pageable"],
+            "decoded_GiBps_pinned": round(e2e["pinned"] * n * 1024 / disk, 3),
+            "matches_device_path": ok,
+            "note": "host src (%.2f GB) + handles + expected CRCs -> descriptors, value offsets and "
+                    "%.2f GB of decoded values in host memory: 64 MiB src chunks, chunk k + 1's H2D "
+                    "under chunk k's values going back (a copy kernel into the mapped out_vals when "
+                    "it is page-locked, else into page-locked staging that host threads copy on), "
+                    "caller-owned output buffers reused.  value: "
+                    "all host buffers in memory allocated page-locked; pageable also given"
+                    % (host_src.size / 1e9, n * 1024 / 1e9)}
 
 
 def run_c4(a, world, rank, local, dev, codec):
